@@ -66,7 +66,7 @@ def _needs_eight_bit(model: Model) -> None:
         raise ValueError("this model has no matrix that can be held in fp8 (those of attention and of SwiGLU feed-forwards can)")
 
 
-def packed_weight_budget(model: Model, dtype: torch.dtype, max_tokens: int, device: torch.device) -> int:
+def packed_weight_budget(model: Model, dtype: torch.dtype, max_tokens: int, device: torch.device, eight_bit: bool = False) -> int:
     """Bytes that the packed copies of the bfloat16 matrices may take (the few-row products stream
     a packed copy a quarter faster and the tiled product of prompts reads nothing else; the
     row-major one serves what has no copy): what is free on the GPU now,
@@ -80,15 +80,15 @@ def packed_weight_budget(model: Model, dtype: torch.dtype, max_tokens: int, devi
     with torch.cuda.device(device):
         free, total = torch.cuda.mem_get_info()
         free += torch.cuda.memory_reserved() - torch.cuda.memory_allocated()      # what torch holds but does not use
-    return max(0, int(free - 0.15 * total) - _own_bytes(model, dtype, max_tokens))
+    return max(0, int(free - 0.15 * total) - _own_bytes(model, dtype, max_tokens, eight_bit))
 
 
-def _own_bytes(model: Model, dtype: torch.dtype, max_tokens: int) -> int:
-    """Bytes of the matrices and the key/value cache."""
+def _own_bytes(model: Model, dtype: torch.dtype, max_tokens: int, eight_bit: bool = False) -> int:
+    """Bytes of the matrices, with eight_bit those that may be in 8 bits, and the key/value cache."""
     element = torch.empty((), dtype=dtype).element_size()
     elements = sum(math.prod(spec.shape) for spec in model.tensor_specs() if spec.kind in ("matrix", "table"))
-    return element * (elements + max_tokens * sum(kv.n_kv_heads * (kv.head_dim + (kv.value_dim if kv.values else 0))
-                                                  for kv, _ in model.cache_needs() if kv is not None))
+    cache = max_tokens * sum(kv.n_kv_heads * (kv.head_dim + (kv.value_dim if kv.values else 0)) for kv, _ in model.cache_needs() if kv is not None)
+    return element * (elements + cache) - (model.eight_bit_saving() if eight_bit else 0)
 
 
 def _packing(rt: Runtime, model: Model, max_tokens: int, pack_weights: Optional[bool]) -> None:
@@ -96,12 +96,12 @@ def _packing(rt: Runtime, model: Model, max_tokens: int, pack_weights: Optional[
     Experts, of which a token is multiplied with a few, get what the other matrices' copies leave, less room for a second
     engine like this one without copies of its experts."""
     rt.pack_weights = pack_weights is not False and rt.dtype == torch.bfloat16
-    rt.pack_budget = packed_weight_budget(model, rt.dtype, max_tokens, rt.device) if pack_weights is None else None
+    rt.pack_budget = packed_weight_budget(model, rt.dtype, max_tokens, rt.device, rt.eight_bit) if pack_weights is None else None
     rt.expert_budget = 0
     if rt.pack_weights and model.expert_elements():
-        free = packed_weight_budget(model, rt.dtype, max_tokens, rt.device) if rt.pack_budget is None else rt.pack_budget
-        others = model.packable_bytes()
-        rt.expert_budget = max(0, free - 2 * others - _own_bytes(model, rt.dtype, max_tokens))
+        free = packed_weight_budget(model, rt.dtype, max_tokens, rt.device, rt.eight_bit) if rt.pack_budget is None else rt.pack_budget
+        others = model.packable_bytes(rt.eight_bit)
+        rt.expert_budget = max(0, free - 2 * others - _own_bytes(model, rt.dtype, max_tokens, rt.eight_bit))
         if rt.pack_budget is not None:
             rt.pack_budget -= rt.expert_budget
 

@@ -216,9 +216,13 @@ class Model:
         """How many products may hold their matrix in 8 bits (each layer once)."""
         return sum(p.eight_bit_matrices() for p in self.layers + self.stream_parts)
 
-    def packable_bytes(self) -> int:
-        """What the packed copies of all matrices but the experts' take (each layer once)."""
-        return sum(p.packable_bytes() for p in self.layers + self.stream_parts) + self.head.packable_bytes()
+    def eight_bit_saving(self) -> int:
+        """Bytes by which those matrices are smaller so than in bfloat16 (each layer once)."""
+        return sum(p.eight_bit_saving() for p in self.layers + self.stream_parts)
+
+    def packable_bytes(self, eight_bit: bool = False) -> int:
+        """What the packed copies of all matrices but the experts' take (each layer once).  eight_bit: where those that may are held in 8 bits, without a copy."""
+        return sum(p.packable_bytes(eight_bit) for p in self.layers + self.stream_parts) + self.head.packable_bytes()
 
     def packed_weight_bytes(self) -> int:
         """Bytes of device memory that the packed second copies of the matrices take (each layer once)."""

@@ -3101,6 +3101,11 @@ def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return codes, powers
 
 
+def block_weight_bytes(N: int, K: int) -> int:
+    """What a BlockWeight of a matrix [N, K] takes: blocks of 64 rows and 128 values with a byte a strip of 16 rows."""
+    return -(-N // 64) * _blocks8(K) * (64 * BLOCK8 + 4)
+
+
 def block_weight(codes: torch.Tensor, powers: torch.Tensor, gate_rows: int = 0) -> BlockWeight:
     """The matrix of codes [N, K] float8_e4m3fn and powers [ceil(N / 128), ceil(K / 128)] float8_e8m0fnu (quantize_weight) as the products take it.  gate_rows: it is
     a gate matrix on top of an up matrix of gate_rows rows each (a multiple of 16), and products with it are silu(gate) * up."""

@@ -153,14 +153,15 @@ class Part:
                 total += sum(x.packed_bytes() for x in v if isinstance(x, Part))
         return total
 
-    def packable_bytes(self) -> int:
-        """What the packed copies of all matrices of this part and its sub-parts take but those of experts, bound or not."""
+    def packable_bytes(self, eight_bit: bool = False) -> int:
+        """What the packed copies of all matrices of this part and its sub-parts take but those of experts, bound or not.  eight_bit: under a Runtime
+        that holds those in 8 bits whose parts allow it, which have no such copy."""
         total = 0
         for v in vars(self).values():
             if isinstance(v, Part):
-                total += v.packable_bytes()
+                total += v.packable_bytes(eight_bit)
             elif isinstance(v, (list, tuple)):
-                total += sum(x.packable_bytes() for x in v if isinstance(x, Part))
+                total += sum(x.packable_bytes(eight_bit) for x in v if isinstance(x, Part))
         return total
 
     def eight_bit_matrices(self) -> int:
@@ -171,6 +172,16 @@ class Part:
                 total += v.eight_bit_matrices()
             elif isinstance(v, (list, tuple)):
                 total += sum(x.eight_bit_matrices() for x in v if isinstance(x, Part))
+        return total
+
+    def eight_bit_saving(self) -> int:
+        """Bytes by which the matrices of this part and its sub-parts that may be held in 8 bits are smaller so than in bfloat16 (small ones are larger: blocks of 64 rows and 128 values)."""
+        total = 0
+        for v in vars(self).values():
+            if isinstance(v, Part):
+                total += v.eight_bit_saving()
+            elif isinstance(v, (list, tuple)):
+                total += sum(x.eight_bit_saving() for x in v if isinstance(x, Part))
         return total
 
     def expert_elements(self) -> int:

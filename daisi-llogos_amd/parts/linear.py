@@ -96,8 +96,11 @@ class Linear(Part):
     def eight_bit_matrices(self) -> int:
         return int(self.eight_bit)
 
-    def packable_bytes(self) -> int:
-        return K.packed_weight_bytes(self.total_out, self.in_features)
+    def eight_bit_saving(self) -> int:
+        return 2 * self.matrix_elements() - K.block_weight_bytes(self.total_out, self.in_features) if self.eight_bit else 0
+
+    def packable_bytes(self, eight_bit: bool = False) -> int:
+        return 0 if eight_bit and self.eight_bit else K.packed_weight_bytes(self.total_out, self.in_features)
 
     def _packed_rows(self, rows_out: Optional[int]) -> Optional[K.PackedWeight]:
         if self.packed is None or rows_out is None:
