@@ -112,6 +112,12 @@ class Linear(Part):
         total = self.block.bytes() if self.block is not None else self.weight.numel() * self.weight.element_size() if self.weight is not None else 0
         return total + (self.bias.numel() * self.bias.element_size() if self.bias is not None else 0)
 
+    def _whole_block(self) -> K.BlockWeight:
+        """The matrix in 8 bits, for its rows as they are stacked."""
+        if self.block.gate_rows:
+            raise K.KernelError("a gate and up matrix in 8 bits gives silu(gate) * up only (gated_product)")
+        return self.block
+
     def _block_product(self, a, w: K.BlockWeight, gated_input: bool = False, bias: Optional[torch.Tensor] = None, **form):
         if isinstance(a, NormedRows):
             a = a.tensor()
@@ -128,9 +134,10 @@ class Linear(Part):
         (NormedRows), which the product on the packed copy then applies to its result; of a matrix in 8 bits it may
         be rows in 8 bits, and the result is bfloat16 or, with `f32_ok`, maybe float32."""
         if self.block is not None:
-            some = self.block if rows_out is None else self.block.rows(rows_out)
+            whole = self._whole_block()
+            some = whole if rows_out is None else whole.rows(rows_out)
             if some is None:
-                return self._block_product(a, self.block, swiglu_input)[:, :rows_out].contiguous()
+                return self._block_product(a, whole, swiglu_input)[:, :rows_out].contiguous()
             return self._block_product(a, some, swiglu_input, sums_ok=f32_ok)
         if isinstance(a, NormedRows):
             pw = self._packed_rows(rows_out)
@@ -209,7 +216,7 @@ class Linear(Part):
                 rows_out: Optional[int] = None) -> torch.Tensor:
         """a [M, in] -> [M, out]; `rows_out` uses only the first rows of the stacked matrix."""
         if self.block is not None:
-            return self._block_product(a, self.block, bias=self.bias)[:, :rows_out].to(out_dtype or self.rt.dtype).contiguous()
+            return self._block_product(a, self._whole_block(), bias=self.bias)[:, :rows_out].to(out_dtype or self.rt.dtype).contiguous()
         w = self.weight if rows_out is None else self.weight[:rows_out]
         b = self.bias if (self.bias is None or rows_out is None) else self.bias[:rows_out]
         return K.gemm(a, w, b, out_dtype or self.rt.dtype, packed=self._packed_rows(rows_out))

@@ -123,3 +123,14 @@ def test_a_model_that_fits_in_8_bits_alone_keeps_its_copies(monkeypatch):
     rt = base.Runtime(torch.device("cpu"), torch.bfloat16, eight_bit=True)
     step._packing(rt, model, 64, None)
     assert rt.pack_budget == free - own >= model.packable_bytes(True) == model.head.packable_bytes()
+
+
+@pytest.mark.parametrize("call", [lambda l, a: l.product(a), lambda l, a: l.product(a, rows_out=64), lambda l, a: l.product(a, f32_ok=True), lambda l, a: l.forward(a)])
+@pytest.mark.parametrize("rows", [lambda: torch.zeros(3, 128, dtype=torch.bfloat16), lambda: torch.zeros(3, 128), lambda: K.BlockRows(3, 128, torch.empty(0))])
+def test_gate_and_up_in_8_bits_give_their_product_only(call, rows):
+    """A stacked gate and up matrix in 8 bits lies in the order of silu(gate) * up: the rows [gate | up] that product() and forward() are for cannot be had of it."""
+    linear = importlib.import_module("daisi-llogos_amd.parts.linear").Linear(["g", "u"], 128, [64, 64], gated=True, eight_bit=True)
+    linear.rt = base.Runtime(torch.device("cpu"), torch.bfloat16, eight_bit=True)
+    linear.block = K.BlockWeight(torch.zeros(128 * 64, dtype=torch.bfloat16), torch.ones(2, 1, 4, dtype=torch.uint8), 128, 128, 64)
+    with pytest.raises(K.KernelError, match="gated_product"):
+        call(linear, rows())
