@@ -2945,6 +2945,7 @@ BLOCK8 = 128                # values of a block along k (and rows of a matrix's 
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
 GATED_NORMS_MAX_WIDTH = 16384
+_MOST8 = (1 << 31) - 256    # rows, values of a row and parts: the kernels count them, rounded up to whole blocks, in 32 bits
 
 
 def _blocks8(k: int) -> int:
@@ -3052,6 +3053,8 @@ def quantize_rows(a: torch.Tensor, gated: bool = False) -> BlockRows:
     code, stride, index = _dt(a), wide if a.is_contiguous() else _row_stride(a, "quantize_rows"), a.get_device()
     if parts != 1 and (parts < 1 or code != F32):
         raise KernelError("quantize_rows: parts are float32")
+    if M > _MOST8 or wide > (2 * _MOST8 if gated else _MOST8) or parts > _MOST8:
+        raise KernelError("quantize_rows: 2^31 - 256 rows, values and parts at most")
     if wide <= 0 or (gated and wide % 2):
         raise KernelError("quantize_rows: gate and up must be equally wide")
     if index < 0:
@@ -3073,6 +3076,7 @@ def block_rows(codes: torch.Tensor, powers: torch.Tensor) -> BlockRows:
     M, K = codes.shape
     _need(K > 0 and powers.dtype == _E8M0 and tuple(powers.shape) == (M, _blocks8(K)) and powers.device == codes.device,
           "block_rows: powers must be float8_e8m0fnu [M, ceil(K / 128)] beside the codes")
+    _need(max(M, K) <= _MOST8, "block_rows: 2^31 - 256 rows and values at most")
     _need(codes.is_cuda, "block_rows: codes must be on the GPU")
     if codes.get_device() != _current_device():
         with torch.cuda.device(codes.device):
@@ -3091,6 +3095,7 @@ def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _need(isinstance(w, torch.Tensor) and w.dim() == 2 and w.numel() > 0, "quantize_weight: w must be [N, K]")
     N, K = w.shape
     code, stride = _dt(w), _row_stride(w, "quantize_weight")
+    _need(max(N, K) <= _MOST8, "quantize_weight: 2^31 - 256 rows and values at most")
     _need(w.is_cuda, "quantize_weight: w must be on the GPU")
     if w.get_device() != _current_device():
         with torch.cuda.device(w.device):
@@ -3114,6 +3119,7 @@ def block_weight(codes: torch.Tensor, powers: torch.Tensor, gate_rows: int = 0) 
     blocks = _blocks8(K)
     _need(powers.dtype == _E8M0 and tuple(powers.shape) == (_blocks8(N), blocks) and powers.device == codes.device,
           "block_weight: powers must be float8_e8m0fnu [ceil(N / 128), ceil(K / 128)] beside the codes")
+    _need(max(N, K) <= _MOST8, "block_weight: 2^31 - 256 rows and values at most")
     _need(gate_rows == 0 or (gate_rows > 0 and gate_rows % 16 == 0 and N == 2 * gate_rows), "block_weight: gate and up of a multiple of 16 rows each")
     _need(codes.is_cuda, "block_weight: codes must be on the GPU")
     if codes.get_device() != _current_device():
@@ -3169,6 +3175,8 @@ def gemm_blocks(a, w: BlockWeight, bias: Optional[torch.Tensor] = None, form: in
     quantize_rows, the single-token attention) may be given those, [M, N] of the few-row kernels and of up to 64 rows, [parts, M, N] of a product in parts of k.  (Results are 1.5e-5 of their size off before they are
     rounded: the matrix cores' sums of 8-bit products, csrc/gemm_blocks.hip.  So no float32 ones.)  form: 0, the one of the least
     cost, or that of llogos_gemm_blocks."""
+    if not 0 <= form < 1 << 31:
+        raise KernelError("gemm_blocks: there is no such form")
     if isinstance(a, torch.Tensor) and a.dtype == torch.bfloat16 and a.dim() == 2:
         return _gemm_blocks_of_rows(a, w, bias, form, out_dtype, sums_ok)
     if not isinstance(a, BlockRows) or not isinstance(w, BlockWeight):
@@ -3229,12 +3237,16 @@ def gated_norms(x: torch.Tensor, a: Optional[torch.Tensor], eps: float, post_w: 
     a_code, a_at, parts, part_stride = F32, None, 1, 0
     if H <= 0:
         raise KernelError("gated_norms: rows of no values")
+    if T > _MOST8:
+        raise KernelError("gated_norms: 2^31 - 256 rows at most")
     if a is not None:
         a_code, a_at = _dt(a), a.data_ptr()
         if a.shape != shape:
             parts, part_stride = (0, 0) if a.dim() == 2 else _parts(a)
             if parts < 1 or a.shape[-2:] != shape or (parts > 1 and a_code != F32):
                 raise KernelError("gated_norms: a must have x's shape; parts are float32")
+            if parts > _MOST8:
+                raise KernelError("gated_norms: 2^31 - 256 parts at most")
         if not a.is_contiguous() or a.get_device() != index:
             raise KernelError("gated_norms: a must be contiguous, beside x")
     elif post_w is not None or gate is not None:
