@@ -18,6 +18,7 @@ struct BlocksCall {
     float* sums;                     // [parts][M][64 ceil(N / 64)] of a product in parts of k; [M][N] of the few-row kernels without out
     size_t scale_stride;
     int M, N, blocks, ldo;
+    bool once;                       // wp will not be in the last-level cache when it is read next
 };
 
 __device__ __forceinline__ i32x8_8 two_pieces(u32x4_8 a, u32x4_8 b) {

@@ -261,7 +261,7 @@ LLOGOS_EXPORT int llogos_gemm_blocks_plan(int M, int N, int K, int gated, int un
 }
 
 // a: codes [M][128 blocks] (16-byte aligned), a_scales [blocks][scale_stride]; wp, w_scales: a packed matrix of N rows (gated: gate and up, packed
-// with gate_rows = N / 2); out [M][ldo] bfloat16 of N columns, gated N / 2; bias float32 [N] or null (gated: none).  form: 1, the few-row
+// with gate_rows = N / 2); gated: 0 or 1, and 2 more where wp comes from memory (BlocksCall: once); out [M][ldo] bfloat16 of N columns, gated N / 2; bias float32 [N] or null (gated: none).  form: 1, the few-row
 // kernels; 1,000,000 n + 10,000 g + 100 t + p, tiles of 16 t tokens with g K groups in p parts, n > 0: the row tiles from the n-th on in tiles of half as many
 // tokens.  sums: of more than one part.
 // out null with sums: the float32 sums are the result, for a consumer that takes them ([M][N] of the few-row kernels, or a part's or more's as they are, rows 64 ceil(N / 64) apart; no bias, not gated).  rows8 (instead of out; gated products in tiles of one K group and one part): the result in 8 bits, codes [M][128 ceil(N / 256)] (16-byte aligned) and
@@ -271,6 +271,9 @@ LLOGOS_EXPORT int llogos_gemm_blocks(void* out, const unsigned char* a, const un
                                      unsigned char* rows8, unsigned char* rows8_scales, hipStream_t stream) {
     if (M <= 0 || N <= 0 || K <= 0 || (out && rows8) || (rows8 == nullptr) != (rows8_scales == nullptr) || !a || !a_scales || !wp || !w_scales || scale_stride < M || units < 8) return LLOGOS_BAD_ARGUMENT;
     if (((uintptr_t)a | (uintptr_t)wp) & 15 || ((uintptr_t)w_scales & 3) || ((uintptr_t)a_scales & 3) || ((uintptr_t)sums & 15)) return LLOGOS_BAD_ARGUMENT;
+    if (gated < 0 || gated > 3) return LLOGOS_BAD_ARGUMENT;
+    const bool once = (gated & 2) != 0;
+    gated &= 1;
     if (gated ? (N % 32 || bias || (out && ldo < N / 2)) : out && ldo < N) return LLOGOS_BAD_ARGUMENT;
     if (!out && !rows8 && (form >= 1000000 || !sums || gated || bias)) return LLOGOS_BAD_ARGUMENT;
     if (rows8 && (!gated || form == 1 || ((uintptr_t)rows8 & 15))) return LLOGOS_BAD_ARGUMENT;
@@ -278,7 +281,7 @@ LLOGOS_EXPORT int llogos_gemm_blocks(void* out, const unsigned char* a, const un
     BlocksCall c{};
     c.rows8 = rows8, c.rows8_scales = rows8_scales;
     c.out = (bf16_t*)out, c.a = a, c.a_scales = a_scales, c.wp = wp, c.w_scales = w_scales, c.bias = bias, c.sums = sums, c.scale_stride = (size_t)scale_stride;
-    c.M = M, c.N = N, c.blocks = (K + kBlock8 - 1) / kBlock8, c.ldo = ldo;
+    c.M = M, c.N = N, c.blocks = (K + kBlock8 - 1) / kBlock8, c.ldo = ldo, c.once = once;
     if (form == 1) return launch_few_rows(c, gated != 0, units, stream);
     return launch_blocks_tiles(c, gated != 0, form / 100 % 100, form / 10000 % 100, form / 1000000, form % 100, stream);
 }

@@ -472,12 +472,13 @@ static int launch_tiles_end(const BlocksCall& c, bool gated, int n_full, int par
         if constexpr (KS == 1) return gated && parts == 1 ? launch_tiles_kernel<TM, TS, KS, END_ROWS8>(c, n_full, 1, stream) : LLOGOS_BAD_ARGUMENT;
         else return LLOGOS_BAD_ARGUMENT;
     }
-    // w goes past the L2 where one tile covers the tokens, in four K groups where four do, of matrices of 64 MB and more, of which a model's few do not stay in the
-    // 256 MB last-level cache until the next step (us: 64 x 14,336 x 4,096 gated in two groups 25.5 / past it 23.3.  61 x 4,096 x 14,336, 59 MB, in four groups and parts
-    // 21.3 / 20.7 from memory, but 16.8 / 20.1 from that cache.  Where more tiles take the same rows of w at different times they are read again: 512 x
+    // w goes past the L2 where one tile covers the tokens, in four K groups where four do, if the caller says that it comes from memory: that its program reads more
+    // than the 256 MB last-level cache holds before it reads w again (us: 64 x 14,336 x 4,096 gated in two groups 25.5 / past it 23.3, 61 x 4,096 x 14,336 in four groups and
+    // parts 21.3 / 20.7 from memory, but 16.8 / 20.1 from that cache; a step of 64 tokens of the 8B sizes, 8.0 GB, 3,240 / 3,110, of one such layer and a small head,
+    // 222 MB, 163 / 163.  Where more tiles take the same rows of w at different times they are read again: 512 x
     // 14,336 x 4,096 in two groups 94 / 102)
     const int m_tiles = (c.M + 16 * TM - 1) / (16 * TM);
-    const bool once = KS > 1 && (m_tiles == 1 || (KS == 4 && m_tiles <= 4)) && (double)c.N * c.blocks * kBlock8 >= 64e6;
+    const bool once = KS > 1 && c.once && (m_tiles == 1 || (KS == 4 && m_tiles <= 4));
 #define TILES(TS_, END, PARTS) (KS > 1 && once ? launch_tiles_kernel<TM, TS_, KS, END, (KS > 1)>(c, n_full, PARTS, stream) : launch_tiles_kernel<TM, TS_, KS, END>(c, n_full, PARTS, stream))
     if (parts == 1 && c.out != nullptr) return gated ? TILES(TS, END_GATED, 1) : TILES(TS, END_PLAIN, 1);
     if (TS > 0) return LLOGOS_BAD_ARGUMENT;                  // (half tiles have no parts)

@@ -186,6 +186,11 @@ class Model:
             self.head.bind_shared(self.embed_table, rt)      # one allocation serves both
         else:
             self.head.bind(get, rt)
+        if rt.eight_bit:
+            parts = self.layers + self.stream_parts
+            always = sum(p.weight_bytes() for p in parts + [self.head]) > K.LAST_LEVEL_CACHE
+            for p in parts:
+                p.matrices_come_from_memory(always)
 
     def describe(self) -> str:
         """One line about the built model, from its own parts: layers, widths, vocabulary, and the

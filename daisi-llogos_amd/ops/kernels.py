@@ -2941,6 +2941,7 @@ def measure_mfma_rate(iters: int = 20000, blocks_per_unit: int = 2, device="cuda
 # ----------------------------------------------------------------------------
 # numbers in 8 bits: rows of activations and matrices with a power of two for each block of 128 values along k (csrc/blocks8.h)
 
+LAST_LEVEL_CACHE = 256 << 20     # bytes, behind all units of the GPU
 BLOCK8 = 128                # values of a block along k (and rows of a matrix's tile)
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
@@ -3005,11 +3006,12 @@ class BlockRows:
 
 class BlockWeight:
     """A matrix [N, K] in 8 bits in the order in which the matrix cores take it: e4m3 codes (data, as PackedWeight holds pairs of them) and the powers of two of
-    its tiles of 128 x 128 by strips of 16 rows (scales).  gate_rows > 0: [gate; up] of gate_rows rows each, for silu(gate) * up."""
-    __slots__ = ("data", "scales", "N", "K", "gate_rows")
+    its tiles of 128 x 128 by strips of 16 rows (scales).  gate_rows > 0: [gate; up] of gate_rows rows each, for silu(gate) * up.  once: the program
+    reads more than LAST_LEVEL_CACHE bytes before it reads this matrix again, so that it comes from memory each time."""
+    __slots__ = ("data", "scales", "N", "K", "gate_rows", "once")
 
-    def __init__(self, data: torch.Tensor, scales: torch.Tensor, N: int, K: int, gate_rows: int = 0):
-        self.data, self.scales, self.N, self.K, self.gate_rows = data, scales, N, K, gate_rows
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, N: int, K: int, gate_rows: int = 0, once: bool = False):
+        self.data, self.scales, self.N, self.K, self.gate_rows, self.once = data, scales, N, K, gate_rows, once
 
     @property
     def out_features(self) -> int:
@@ -3022,7 +3024,7 @@ class BlockWeight:
             return self
         if n <= 0 or n > self.N or n % 64 or self.gate_rows:
             return None
-        return BlockWeight(self.data[:n // 64 * _blocks8(self.K) * (32 * BLOCK8)], self.scales[:n // 64], n, self.K)
+        return BlockWeight(self.data[:n // 64 * _blocks8(self.K) * (32 * BLOCK8)], self.scales[:n // 64], n, self.K, 0, self.once)
 
     def bytes(self) -> int:
         return self.data.numel() * self.data.element_size() + self.scales.numel()
@@ -3111,9 +3113,10 @@ def block_weight_bytes(N: int, K: int) -> int:
     return -(-N // 64) * _blocks8(K) * (64 * BLOCK8 + 4)
 
 
-def block_weight(codes: torch.Tensor, powers: torch.Tensor, gate_rows: int = 0) -> BlockWeight:
+def block_weight(codes: torch.Tensor, powers: torch.Tensor, gate_rows: int = 0, once: bool = False) -> BlockWeight:
     """The matrix of codes [N, K] float8_e4m3fn and powers [ceil(N / 128), ceil(K / 128)] float8_e8m0fnu (quantize_weight) as the products take it.  gate_rows: it is
-    a gate matrix on top of an up matrix of gate_rows rows each (a multiple of 16), and products with it are silu(gate) * up."""
+    a gate matrix on top of an up matrix of gate_rows rows each (a multiple of 16), and products with it are silu(gate) * up.  once: see BlockWeight; the
+    results are the same."""
     _need(codes.dtype == _E4M3 and codes.dim() == 2 and codes.numel() > 0, "block_weight: codes must be float8_e4m3fn [N, K]")
     N, K = codes.shape
     blocks = _blocks8(K)
@@ -3124,7 +3127,7 @@ def block_weight(codes: torch.Tensor, powers: torch.Tensor, gate_rows: int = 0) 
     _need(codes.is_cuda, "block_weight: codes must be on the GPU")
     if codes.get_device() != _current_device():
         with torch.cuda.device(codes.device):
-            return block_weight(codes, powers, gate_rows)
+            return block_weight(codes, powers, gate_rows, once)
     rows = codes.view(torch.uint8)
     if K != blocks * BLOCK8 or not rows.is_contiguous() or rows.data_ptr() % 16:
         full = torch.zeros((N, blocks * BLOCK8), dtype=torch.uint8, device=codes.device)
@@ -3133,7 +3136,7 @@ def block_weight(codes: torch.Tensor, powers: torch.Tensor, gate_rows: int = 0) 
     data = pack_weights(rows.view(torch.bfloat16), gate_rows).data
     scales = torch.empty((-(-N // 64), blocks, 4), dtype=torch.uint8, device=codes.device)
     _check(_lib().llogos_strip_scales(_p(scales), _p(powers.view(torch.uint8).contiguous()), N, K, int(gate_rows), _stream()), "block_weight")
-    return BlockWeight(data, scales, N, K, int(gate_rows))
+    return BlockWeight(data, scales, N, K, int(gate_rows), bool(once))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -3209,7 +3212,7 @@ def gemm_blocks(a, w: BlockWeight, bias: Optional[torch.Tensor] = None, form: in
     out = sums if only_sums else BlockRows(M, width, rows) if fused else rows.new_empty((M, width), dtype=torch.bfloat16)
     at, eight_at = rows.data_ptr(), out.buffer.data_ptr() if fused else None
     _check(_lib().llogos_gemm_blocks(None if fused or only_sums else out.data_ptr(), at, at + M * a.blocks * BLOCK8, a.stride, data.data_ptr(), w.scales.data_ptr(),
-                                     None if bias is None else bias.data_ptr(), M, N, K, width, gated, form,
+                                     None if bias is None else bias.data_ptr(), M, N, K, width, gated + 2 if w.once else gated, form,
                                      None if sums is None else sums.data_ptr(), units, eight_at, eight_at + M * out.blocks * BLOCK8 if fused else None,
                                      _stream_of(index)), "gemm_blocks")
     return out if fused or not eight else quantize_rows(out)

@@ -174,6 +174,13 @@ class Part:
                 total += sum(x.eight_bit_matrices() for x in v if isinstance(x, Part))
         return total
 
+    def matrices_come_from_memory(self, always: bool) -> None:
+        """Tell this part's matrices and its sub-parts' whether the model's together are more than the last-level cache holds until the next step (ops.kernels.BlockWeight.once)."""
+        for v in vars(self).values():
+            for x in v if isinstance(v, (list, tuple)) else (v,):
+                if isinstance(x, Part):
+                    x.matrices_come_from_memory(always)
+
     def eight_bit_saving(self) -> int:
         """Bytes by which the matrices of this part and its sub-parts that may be held in 8 bits are smaller so than in bfloat16 (small ones are larger: blocks of 64 rows and 128 values)."""
         total = 0

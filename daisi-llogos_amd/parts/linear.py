@@ -96,6 +96,10 @@ class Linear(Part):
     def eight_bit_matrices(self) -> int:
         return int(self.eight_bit)
 
+    def matrices_come_from_memory(self, always: bool) -> None:
+        if self.block is not None:
+            self.block.once = always
+
     def eight_bit_saving(self) -> int:
         return 2 * self.matrix_elements() - K.block_weight_bytes(self.total_out, self.in_features) if self.eight_bit else 0
 

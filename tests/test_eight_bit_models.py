@@ -134,3 +134,32 @@ def test_gate_and_up_in_8_bits_give_their_product_only(call, rows):
     linear.block = K.BlockWeight(torch.zeros(128 * 64, dtype=torch.bfloat16), torch.ones(2, 1, 4, dtype=torch.uint8), 128, 128, 64)
     with pytest.raises(K.KernelError, match="gated_product"):
         call(linear, rows())
+
+
+def test_whether_matrices_come_from_memory(monkeypatch):
+    """A model that is larger than the last-level cache says so to its matrices in 8 bits, whatever their own size is; a smaller one does not."""
+    config = peponex_configs.PEP_C
+    for small, large in ((1 << 10, False), (1 << 30, True)):
+        model, _ = bound8(monkeypatch, config, 1 << 40)
+        held = sum(p.weight_bytes() for p in model.layers + model.stream_parts) + model.head.weight_bytes()
+        assert (1 << 10) < held < (1 << 30)
+        monkeypatch.setattr(K, "LAST_LEVEL_CACHE", small)
+        model, _ = bound8(monkeypatch, config, 1 << 40)
+        blocks = [l.block for layer in model.layers for l in linears(layer) if l.block is not None]
+        assert blocks and all(b.once is not large for b in blocks)
+    w = K.BlockWeight(torch.zeros(2 * 64 * 64, dtype=torch.bfloat16), torch.ones(2, 1, 4, dtype=torch.uint8), 128, 128, once=True)
+    assert w.rows(64).once and w.rows(128).once
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [0, 20401, 40401, 40403, 20805, 10401, 1])
+@pytest.mark.parametrize("M", [20, 61, 130, 300])
+@pytest.mark.parametrize("gate_rows", [0, 160])
+def test_a_matrix_from_memory_gives_the_same(form, M, gate_rows):
+    g = torch.Generator(device="cuda").manual_seed(form + M)
+    a, w = torch.randn(M, 1600, generator=g, device="cuda"), torch.randn(320, 1600, generator=g, device="cuda")
+    rows, matrix = K.quantize_rows(a), K.quantize_weight(w)
+    one, other = (K.block_weight(*matrix, gate_rows=gate_rows, once=o) for o in (False, True))
+    assert other.once and not one.once
+    assert torch.equal(K.gemm_blocks(rows, one, form=form), K.gemm_blocks(rows, other, form=form))
+    assert torch.equal(K.gemm_blocks(rows, one, form=form, sums_ok=True), K.gemm_blocks(rows, other, form=form, sums_ok=True))
