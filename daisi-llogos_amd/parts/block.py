@@ -15,7 +15,7 @@ from typing import Callable, List, Optional, Tuple
 import torch
 
 from .base import Block, FeedForward, LayerCache, Mixer, Norm, NormedAhead, Part, Residual, Runtime, StepContext, TensorSpec, mark, register_block
-from .norm import RMSNorm, add_normed
+from .norm import RMSNorm, add_normed, add_normed_block_rows
 
 
 @register_block("pre_norm")
@@ -149,7 +149,9 @@ class SandwichBlock(Block):
             rows, delta = self._close(x, a, self.post_mixer_norm, next_norm, True)
             mark(ctx, "norm")
             return x, (delta if rows is None else NormedAhead(rows, next_norm))
-        rows, delta = self._close(x, a, self.post_mixer_norm, self.ffn_norm, self.ffn_conv is not None)
+        delta, rows = None, add_normed_block_rows(x, a, self.post_mixer_norm, self.ffn_norm) if self.ffn_conv is None and self.ffn.takes_block_rows else None
+        if rows is None:
+            rows, delta = self._close(x, a, self.post_mixer_norm, self.ffn_norm, self.ffn_conv is not None)
         mark(ctx, "norm")
         if rows is None:
             h = self._read(ctx, self.ffn_norm, self.ffn_conv, x, delta, conv2_cache, False)
@@ -360,7 +362,9 @@ class OutputNormBlock(Block):
         mark(ctx, "norm")
         a = self.mixer.forward(ctx, h, cache)
         mark(ctx, "mixer")
-        h = self._close(x, a, self.mixer_norm)
+        h = add_normed_block_rows(x, a, self.mixer_norm, None) if self.ffn is not None and self.ffn.takes_block_rows else None
+        if h is None:
+            h = self._close(x, a, self.mixer_norm)
         mark(ctx, "norm")
         if self.ffn is not None:
             d = self.ffn.forward(ctx, h)

@@ -27,6 +27,15 @@ def add_normed(x: torch.Tensor, out: torch.Tensor, post: Norm, nxt: Optional[Nor
     return NormedAhead(rows, nxt)
 
 
+def add_normed_block_rows(x: torch.Tensor, out: torch.Tensor, post: Norm, nxt: Optional[Norm]) -> Optional[K.BlockRows]:
+    """The stream x (float32, in place) += post(out), and the rows that nxt makes of the completed stream, or without it the stream's own, in 8 bits for the product that
+    reads them next: one kernel where the norms are RMS norms; else None, and x is as it was."""
+    if not isinstance(post, RMSNorm) or not (nxt is None or isinstance(nxt, RMSNorm)) or x.shape[1] > K.GATED_NORMS_MAX_WIDTH:
+        return None
+    return K.gated_norms(x, out, post.eps if nxt is None else nxt.eps, post_w=post.weight, next_w=None if nxt is None else nxt.weight,
+                         out_dtype=torch.float8_e4m3fn, post_eps=post.eps)
+
+
 @register_norm("rmsnorm")
 class RMSNorm(Norm):
     takes_row_squares = True
